@@ -7,14 +7,17 @@
 //     more query heads): scores K Q^T, then outputs V^T P^T with 16 elements of the head as M.  Heads as M fill seven of sixteen rows
 //     in a group of seven; this way takes half the products, accumulators and exponentials.  Probabilities change sides by movmatrix.
 //   * e4m3 numbers become float16 in one instruction for two (exact), and float16 is what is multiplied, not bfloat16: queries
-//     are brought to 2^13 .. 2^14 per head by a power of two, which keeps all their bits, and probabilities keep three bits more
-//     than in bfloat16.
+//     are brought to 2^13 .. 2^14 per head by a power of two, which keeps all their bits.
 //   * keys are read from shared memory 16 bytes at a time as they lie; which of the head's elements stand at which place of a
 //     product's k index is free as long as the queries agree, and so is the order of a tile's keys.
 //   * values are transposed in pairs of bytes by ldmatrix; one byte permute then gives the even and the odd column's pairs, which
 //     are the two halves of a product's 16 rows.
-//   * a block's scale of the keys goes into the exponent's factor, that of the values multiplies the probabilities, relative to
-//     the largest that the warp has met (2^v_top, which comes back at the end).
+//   * a block's scale of the keys goes into the exponent's factor.  Its values are weighed by probabilities that are relative to
+//     the block's own largest one, times 2^7, in float16: eleven bits down to 2^-21 of that one (three more than in bfloat16) and off by
+//     2^-32 of it at most below.  The block's sums join the warp's in float32, times the scale of its values and what its largest
+//     probability is of the warp's, so that neither a weight nor a scale far from other blocks' costs any block its bits: with
+//     both in the float16 numbers, relative to the largest scale the warp had met, a block of 2^-16 of that scale lost bits and one of
+//     2^-25 was 0, whatever its weight.
 // Values of keys that the query does not see are zeroed: what stands behind a request's last token in its page may be anything.
 //
 // With FRESH the kernel starts from the q/k/v product, which qkv_rope_store8 followed by it would do in two launches: it adds up the
@@ -25,8 +28,6 @@
 // launch right ahead started, and the old keys are on their way while the product ends.
 //
 // Every wait on an mbarrier is bounded (tma.cuh); on giving up the block flags *status = 5.
-#include <limits.h>
-
 #include "cache8.cuh"
 #include "mma.cuh"
 #include "tma.cuh"
@@ -42,6 +43,19 @@ __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same with nothing to add to.
+__device__ __forceinline__ void mma_f16_16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// a += x f.x, b += y f.y, in one instruction.
+__device__ __forceinline__ void add_two(float& a, float& b, float x, float y, float2 f) {
+    asm("{\n\t.reg .b64 s, v, f;\n\tmov.b64 s, {%0, %1};\n\tmov.b64 v, {%2, %3};\n\tmov.b64 f, {%4, %5};\n\t"
+        "fma.rn.f32x2 s, v, f, s;\n\tmov.b64 {%0, %1}, s;\n\t}"
+        : "+f"(a), "+f"(b) : "f"(x), "f"(y), "f"(f.x), "f"(f.y));
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     uint32_t r;
@@ -214,7 +228,6 @@ decode_attention8_kernel(const __grid_constant__ CUtensorMap map_cache, const Fr
         m[x][0] = m[x][1] = -INFINITY;
         l[x][0] = l[x][1] = 0.f;
     }
-    int v_top = INT_MIN / 2;                                 // the accumulators are in units of 2^v_top
 
     if (warp == D8_CONSUMERS) {
         // ------------------------------------------------------------ copies
@@ -384,7 +397,7 @@ decode_attention8_kernel(const __grid_constant__ CUtensorMap map_cache, const Fr
                 }
                 const bool whole = kbase >= lo && kbase + 15 <= pos;
                 auto seen = [&](int place) { return kbase + place >= lo && kbase + place <= pos; };
-                float top_of[GROUPS][2];
+                float top_here[GROUPS][2];      // the block's largest scores
                 bool move = false;
 #pragma unroll
                 for (int x = 0; x < GROUPS; ++x) {
@@ -401,36 +414,41 @@ decode_attention8_kernel(const __grid_constant__ CUtensorMap map_cache, const Fr
                         tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 4));
                         tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 8));
                         tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 16));
-                        top_of[x][h] = fmaxf(m[x][h], tm);                  // finite: at least one key is visible
-                        move |= top_of[x][h] > m[x][h];
+                        // (at least one key is visible; a block whose scores have all run to -infinity weighs nothing)
+                        top_here[x][h] = fmaxf(tm, -3e38f);
+                        move |= top_here[x][h] > m[x][h];
                     }
                 }
-                const int ev = (int)(__float_as_uint(sv) >> 23) - 127, top = max(v_top, ev);
-                if (__any_sync(0xffffffffu, move || top > v_top)) {
-                    const float cv = exp2_int(v_top - top);
-                    v_top = top;
+                if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
                     for (int x = 0; x < GROUPS; ++x)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const float c = exp2_quick(m[x][h] - top_of[x][h]), both = c * cv;
-                            m[x][h] = top_of[x][h];
+                            const float top = fmaxf(m[x][h], top_here[x][h]), c = exp2_quick(m[x][h] - top);
+                            m[x][h] = top;
                             l[x][h] *= c;
 #pragma unroll
-                            for (int n = 0; n < CH; ++n) o[x][n][h] *= both, o[x][n][2 + h] *= both;
+                            for (int n = 0; n < CH; ++n) o[x][n][h] *= c, o[x][n][2 + h] *= c;
                         }
                 }
-                const float pv = exp2_int(ev - v_top);
                 uint32_t pb[GROUPS][2];
+                float2 unit[GROUPS];      // what the block's sums are of the warp's
 #pragma unroll
-                for (int x = 0; x < GROUPS; ++x)
+                for (int x = 0; x < GROUPS; ++x) {
+                    // (7: where scores are so large that the difference is rounded, it is 8 at most)
+                    const float from0 = top_here[x][0] - 7.f, from1 = top_here[x][1] - 7.f;
+                    const float of0 = exp2_quick(from0 - m[x][0]), of1 = exp2_quick(from1 - m[x][1]);
+                    unit[x] = make_float2(of0 * sv, of1 * sv);
+                    float p[2][2];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const float p0 = exp2_quick(s[x][2 * j] - m[x][0]), p1 = exp2_quick(s[x][2 * j + 1] - m[x][1]);
-                        l[x][0] += p0;
-                        l[x][1] += p1;
-                        pb[x][j] = transposed(pack_f16(p0 * pv, p1 * pv));
+                        p[j][0] = exp2_quick(s[x][2 * j] - from0);
+                        p[j][1] = exp2_quick(s[x][2 * j + 1] - from1);
+                        pb[x][j] = transposed(pack_f16(p[j][0], p[j][1]));
                     }
+                    l[x][0] = fmaf(p[0][0] + p[1][0], of0, l[x][0]);
+                    l[x][1] = fmaf(p[0][1] + p[1][1], of1, l[x][1]);
+                }
                 uint32_t live[2] = {0xffffffffu, 0xffffffffu};
                 if (!whole)
 #pragma unroll
@@ -455,7 +473,12 @@ decode_attention8_kernel(const __grid_constant__ CUtensorMap map_cache, const Fr
                         const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)b[2 * i]), a1 = e4m3x2_to_f16x2((uint16_t)(b[2 * i] >> 16));
                         const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)b[2 * i + 1]), a3 = e4m3x2_to_f16x2((uint16_t)(b[2 * i + 1] >> 16));
 #pragma unroll
-                        for (int x = 0; x < GROUPS; ++x) mma_f16_16816(o[x][n + i], a0, a1, a2, a3, pb[x][0], pb[x][1]);
+                        for (int x = 0; x < GROUPS; ++x) {
+                            float here[4];
+                            mma_f16_16816_first(here, a0, a1, a2, a3, pb[x][0], pb[x][1]);
+                            add_two(o[x][n + i][0], o[x][n + i][1], here[0], here[1], unit[x]);
+                            add_two(o[x][n + i][2], o[x][n + i][3], here[2], here[3], unit[x]);
+                        }
                     }
                 }
             }
@@ -478,7 +501,6 @@ decode_attention8_kernel(const __grid_constant__ CUtensorMap map_cache, const Fr
         return;
     }
     if (warp < D8_CONSUMERS) {
-        const float unit = exp2_int(v_top);
 #pragma unroll
         for (int x = 0; x < GROUPS; ++x)
 #pragma unroll
@@ -487,7 +509,7 @@ decode_attention8_kernel(const __grid_constant__ CUtensorMap map_cache, const Fr
                 if (g == 0) sm_m[row] = m[x][h], sm_l[row] = l[x][h];
 #pragma unroll
                 for (int n = 0; n < CH; ++n)
-                    *reinterpret_cast<float2*>(sm_o + row * D + 16 * n + 2 * g) = make_float2(o[x][n][h] * unit, o[x][n][2 + h] * unit);
+                    *reinterpret_cast<float2*>(sm_o + row * D + 16 * n + 2 * g) = make_float2(o[x][n][h], o[x][n][2 + h]);
             }
     }
     __syncthreads();

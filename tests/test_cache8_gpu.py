@@ -548,3 +548,29 @@ def test_portions_on_two_streams_at_once():
             call(out)
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("d,H,K", [(128, 8, 2), (64, 4, 4), (128, 24, 2)])
+@pytest.mark.parametrize("tile,splits", [(0, 1), (0, None), (7, 1)])
+@pytest.mark.parametrize("apart,key_scale", [(0, 4.0), (16, 4.0), (20, 4.0), (24, 4.0), (40, 4.0), (100, 4.0), (60, 0.5)])
+def test_a_tile_of_large_values_costs_the_others_no_bits(d, H, K, tile, splits, apart, key_scale):
+    """One tile's values have scales 2^apart above the others'; its keys point away from the queries, so that it has hardly any weight (or,
+    in the last case, little enough that its values still decide)."""
+    P, n = 64, 512
+    pool = Pool([n], K, P, d, seed=41 + d)
+    page = int(pool.table[pool.slots[0], tile])
+    pool.cache[page, 0] = torch.full((K, P, d), -8.0, device="cuda").to(torch.float8_e4m3fn)
+    pool.scales[page, 0] = key_scale
+    pool.scales[page, 1] *= 2.0 ** apart
+    q = torch.randn((1, H, d), generator=pool.g).abs().bfloat16()
+    out = torch.full((1, H, d), math.nan, dtype=torch.bfloat16, device="cuda")
+    pos, seq = batch([1], [n - 1], pool.slots)
+    ops.decode_attention8(q.cuda(), pool.cache, pool.scales, pool.table, seq, pos, out, None, d ** -0.5, splits=splits)
+    rows = pool.rows(pool.slots[0], n)
+    want, size = attention64(q, torch.tensor([n - 1]), rows, None, d ** -0.5)
+    # probabilities are rounded to float16 (2^-11; those below 2^-21 of their block's largest are off by 2^-32 of it, for n keys),
+    # scores and sums in float32, the output to bfloat16 (2^-8); the other tiles' weights are all of the denominator
+    rows[1, :, 64 * tile:64 * (tile + 1)] = 0
+    largest = rows[1].abs().amax((1, 2)).repeat_interleave(H // K, 0)[None, :, None]
+    tolerance = size * (2.0 ** -11 + 2.0 ** -16) + want.abs() * 2.0 ** -8 + largest * n * 2.0 ** -32
+    assert ((out.cpu().double() - want).abs() <= tolerance * 1.01 + 1e-30).all()
