@@ -463,13 +463,24 @@ __device__ __forceinline__ void read_sums(uint32_t tmem, uint32_t (&v)[COLS]) {
     }
 }
 // gated_activation (common.cuh) by the special-function unit's exponential and reciprocal (2^-22 off, which a float32 output shows and a
-// bfloat16 one does not): the accurate forms, of 60 instructions, took as long as the products of a step.
+// bfloat16 one does not): the accurate forms, of 60 instructions, took as long as the products of a step.  Cuts and the rectifier hand NaN
+// on (a block of a number that is not finite is NaN, and what is made of it must be).
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 __device__ __forceinline__ float gated_quick(float g, float u, float neg_alpha_log2, float limit, float shift) {
     if (limit > 0.f) {
-        g = fminf(g, limit);
-        u = fminf(fmaxf(u, -limit), limit);
+        g = min_or_nan(g, limit);
+        u = min_or_nan(max_or_nan(u, -limit), limit);
     }
-    if (neg_alpha_log2 > 0.f) return fmaxf(g, 0.f) * (u + shift);
+    if (neg_alpha_log2 > 0.f) return max_or_nan(g, 0.f) * (u + shift);
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * neg_alpha_log2));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
