@@ -422,6 +422,7 @@ struct MxShape {
     const float* ss;
     int chunks, width;
     float eps;
+    int w_ready;      // (few rows' kernel) W was complete before the predecessor, which rounds rows, passed its own wait
 };
 constexpr int MX_STORE = 0, MX_ADD = 1, MX_GATED = 2;
 
@@ -579,8 +580,9 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
 
     if (warp == 0 || warp == X_WARP) {
         // ---------------------------------------------------- copies
-        // (the weights were written before the predecessor started, see mxfp4_quantise_kernel: only the tokens wait for it)
-        if (warp == X_WARP) pdl_wait();
+        // (w_ready: only the tokens wait.  A kernel that rounds rows lets this one start behind its own wait, so that weights written
+        // ahead of it are there; rounding may be rounding of these very weights where no rounding of tokens stands in between)
+        if (warp == X_WARP || !s.w_ready) pdl_wait();
         uint32_t st = 0, parity = 1;
         while (it.item < items) {
             if (!warp_wait(&empty[st], parity, abort_flag)) break;        // (a fresh barrier's phase ahead of its first counts as over)
@@ -968,6 +970,7 @@ struct MxCall {
     const float* ss;
     int chunks;
     float eps;
+    int w_ready;
 };
 
 // pair: 0, a block for itself; 1, two share a tile (cluster of two).
@@ -975,7 +978,7 @@ template <typename Tile, int TN, int TERMS, typename TO, typename Kernel>
 static int launch_mxfp4(Kernel kernel, int pair, int x_rows, const MxCall& c) {
     const int rows = MX_BM << pair, units = c.sms >> pair;
     const MxShape s{c.T, c.N, c.splits, (c.K + MX_STEP - 1) / MX_STEP, (c.N + rows - 1) / rows, (c.T + TN - 1) / TN,
-                    c.mode, c.alpha, c.limit, c.shift, c.ss, c.chunks, c.K, c.eps};
+                    c.mode, c.alpha, c.limit, c.shift, c.ss, c.chunks, c.K, c.eps, c.w_ready};
     // (a part without a step of k would leave its sums unwritten)
     const int per = (s.k_steps + c.splits - 1) / c.splits;
     const long long items = (long long)s.w_tiles * s.t_tiles * c.splits;
@@ -1149,7 +1152,7 @@ AIR_API int air_mxfp4_linear(const void* x, int dtype, void* memory, const void*
     int rc = dtype == AIR_F32 ? launch_quantise<float>(x, packed, scales, T, K, terms, stream)
              : dtype == AIR_BF16 ? launch_quantise<__nv_bfloat16>(x, packed, scales, T, K, terms, stream) : AIR_ERR_BAD_ARGUMENT;
     if (rc) return rc;
-    MxCall c{packed, scales, w, (const uint8_t*)w_scales, out, T, N, K, splits, sms, status, stream, mode, alpha, limit, shift, nullptr, 0, 0.f};
+    MxCall c{packed, scales, w, (const uint8_t*)w_scales, out, T, N, K, splits, sms, status, stream, mode, alpha, limit, shift, nullptr, 0, 0.f, 1};
     if (join > 1) {
         c.out = at + m.parts, c.splits = join, c.mode = MX_STORE;
         rc = launch_mxfp4_terms<float>(p, terms, c);
@@ -1183,9 +1186,10 @@ AIR_API int air_mxfp4_add_prenorm(float* h, const void* delta, int delta_dtype, 
 
 // air_mxfp4_linear for up to 64 rows that air_mxfp4_add_prenorm has written (ss, `chunks` of them, eps: the norm's scale per row).  k is
 // cut only into the caller's parts (consumers of few rows add them up; a gate/up matrix of so few tiles that parts would pay is small).
+// w_ready: w and w_scales were written ahead of the launch that wrote these rows, and are read while it ends.
 AIR_API int air_mxfp4_linear_normed(const void* packed, const void* scales, const float* ss, int chunks, float eps, const void* w, const void* w_scales,
                                     void* out, int out_dtype, int T, int N, int K, int terms, int splits, int mode, float alpha, float limit,
-                                    float shift, int sms, int* status, cudaStream_t stream) {
+                                    float shift, int sms, int* status, int w_ready, cudaStream_t stream) {
     using namespace air;
     if (!mx_fits(T, K, terms) || T > 64 || N < 1 || splits < 1 || (splits > 1 && (out_dtype != AIR_F32 || mode != MX_STORE)) || sms < 2 || mode < MX_STORE ||
         mode > MX_GATED || (mode == MX_ADD && out_dtype != AIR_F32) || (mode == MX_GATED && N % 2) || !ss || chunks != (K + MXN_CHUNK - 1) / MXN_CHUNK ||
@@ -1194,7 +1198,7 @@ AIR_API int air_mxfp4_linear_normed(const void* packed, const void* scales, cons
     if (T == 0) return 0;
     const MxPlan p = mx_plan(T, N, K, terms, sms);
     const MxCall c{packed, scales, w, (const uint8_t*)w_scales, out, T, N, K, splits, sms, status, stream, mode, alpha, limit, shift,
-                   ss, chunks, eps};
+                   ss, chunks, eps, w_ready};
     AIR_DISPATCH(out_dtype, TO, { return launch_mxfp4_terms<TO>(p, terms, c); });
 }
 

@@ -155,7 +155,7 @@ _SIGNATURES = {
     "air_mxfp4_linear": [c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 7 + [c_float] * 3 + [c_int, c_void_p, c_void_p],
     "air_mxfp4_need": [c_int] * 6 + [c_void_p],
     "air_mxfp4_add_prenorm": [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int] + [c_void_p] * 3 + [c_int] * 3 + [c_void_p],
-    "air_mxfp4_linear_normed": [c_void_p] * 3 + [c_int, c_float] + [c_void_p] * 3 + [c_int] * 7 + [c_float] * 3 + [c_int, c_void_p, c_void_p],
+    "air_mxfp4_linear_normed": [c_void_p] * 3 + [c_int, c_float] + [c_void_p] * 3 + [c_int] * 7 + [c_float] * 3 + [c_int, c_void_p, c_int, c_void_p],
     "air_sample": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                    c_void_p, c_void_p],
 }
@@ -2065,13 +2065,15 @@ def mxfp4_add_prenorm(h, delta, weight, terms, eps):
     return NormedRows4(packed, scales, ss, eps)
 
 
-def mxfp4_linear(x, w, w_scales, out, terms=1, splits=1, status=None, add=False, act=None):
+def mxfp4_linear(x, w, w_scales, out, terms=1, splits=1, status=None, add=False, act=None, w_ready=False):
     """out = x W^T with W [n, k] held in 4 bits (one term: w uint8 [n, k / 2] and w_scales as mxfp4_quantise leaves them) and x
     (float32 or bfloat16 [rows, k]) rounded to the sum of `terms` such numbers inside the call; float32 accumulation.  out
     float32 or bfloat16 [rows, n], or with splits > 1 (up to 64 rows) float32 [splits, rows, n]: partial sums over parts of k.
     add: the product is added to what the float32 out holds.  act = (alpha, limit, shift): rows 2 i and 2 i + 1 of W are gate and up of
     output i, out [rows, n / 2] = the gated activation that gemm_tc describes.  x may be a NormedRows4 of up to 64 rows and `terms` terms:
-    the sums are multiplied by the norm's scale per row first."""
+    the sums are multiplied by the norm's scale per row first.  w_ready (with a NormedRows4): W was written ahead of the launch that
+    wrote x, and is read while that one ends; else W is read when the launch right ahead has ended (plain rows are rounded by a launch of
+    their own, which W is always ahead of)."""
     normed = x if isinstance(x, NormedRows4) else None
     if normed is None:
         _req(x, "x", _FLOATS, (None, None))
@@ -2097,16 +2099,16 @@ def mxfp4_linear(x, w, w_scales, out, terms=1, splits=1, status=None, add=False,
         _req(out, "out", (torch.float32,) if add else _FLOATS, (rows, n))
     if n == 0 or rows == 0:
         return out
-    mode = (2 if act is not None else 1 if add else 0, *(act or SILU), 148, _ptr(status), _stream())
+    mode = (2 if act is not None else 1 if add else 0, *(act or SILU), 148, _ptr(status))
     if normed is not None:
         _check(_get("air_mxfp4_linear_normed")(x.packed.data_ptr(), x.scales.data_ptr(), x.ss.data_ptr(), x.ss.shape[0], x.eps,
                                                w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), _DT[out.dtype], rows, n, k, terms,
-                                               splits, *mode), "mxfp4_linear")
+                                               splits, *mode, 1 if w_ready else 0, _stream()), "mxfp4_linear")
         return out
     memory = empty((_mxfp4_need(rows, n, k, terms, splits)[0],), torch.uint8, x.device)
     global launches
     _check(_get("air_mxfp4_linear")(x.data_ptr(), _DT[x.dtype], memory.data_ptr(), w.data_ptr(), w_scales.data_ptr(), out.data_ptr(),
-                                    _DT[out.dtype], rows, n, k, terms, splits, *mode), "mxfp4_linear")
+                                    _DT[out.dtype], rows, n, k, terms, splits, *mode, _stream()), "mxfp4_linear")
     launches += 1
     return out
 

@@ -155,11 +155,13 @@ class Linear:
 class MXFP4Linear(Linear):
     """A matrix [out, in] held in microscaled 4-bit floating point (17/32 of a byte a number), made from a tensor of 16 or 32 bits;
     every input is rounded to the sum of `terms` such numbers on its way into the product (ops.mxfp4_linear).  One product serves
-    few rows and many: for few, k is split over blocks, and consumers add the partial sums as they do those of 16-bit weights."""
+    few rows and many: for few, k is split over blocks, and consumers add the partial sums as they do those of 16-bit weights.  The
+    matrix is complete once this is made and is not written any more: products read it ahead of what they wait for (w_ready)."""
 
     def __init__(self, weight: torch.Tensor, terms: int, status: Optional[torch.Tensor] = None, gate_up_block: int = 0):
         packed, scales = ops.mxfp4_empty(weight.shape[0], weight.shape[1], 1, weight.device)
         ops.mxfp4_quantise(weight, packed, scales)
+        torch.cuda.current_stream(weight.device).synchronize()
         self._hold(packed[0], scales[0], terms, status, gate_up_block)
 
     def _hold(self, packed, scales, terms, status, gate_up_block=0):
@@ -190,7 +192,8 @@ class MXFP4Linear(Linear):
         return rows <= SMALL_ROWS
 
     def _product(self, x, out, splits=1):
-        return ops.mxfp4_linear(x, self.weight, self.scales, out, terms=self.terms, splits=splits, status=self.status)
+        return ops.mxfp4_linear(x, self.weight, self.scales, out, terms=self.terms, splits=splits, status=self.status,
+                                w_ready=True)
 
     def partial(self, x) -> torch.Tensor:
         return self._product(x, ops.empty((self.parts, x.shape[0], self.out_features), torch.float32, x.device), self.parts) \
@@ -203,7 +206,7 @@ class MXFP4Linear(Linear):
         """The gated activation in the product's epilogue: rows of the matrix are gate and up in turn (make_gate_up)."""
         out = ops.empty((x.shape[0], self.out_features // 2), torch.bfloat16, x.device)
         return ops.mxfp4_linear(x, self.weight, self.scales, out, terms=self.terms, status=self.status,
-                                act=tuple(float(a) for a in act))
+                                act=tuple(float(a) for a in act), w_ready=True)
 
     def adds_into(self, x, residual) -> bool:
         return (residual is not None and x.is_cuda and residual.dtype == torch.float32
@@ -211,7 +214,7 @@ class MXFP4Linear(Linear):
 
     def add_into(self, x, residual) -> None:
         """residual += x W^T, in the product's epilogue."""
-        ops.mxfp4_linear(x, self.weight, self.scales, residual, terms=self.terms, status=self.status, add=True)
+        ops.mxfp4_linear(x, self.weight, self.scales, residual, terms=self.terms, status=self.status, add=True, w_ready=True)
 
     def __call__(self, x: torch.Tensor, out_dtype: torch.dtype, bias=None) -> torch.Tensor:
         if bias is not None:
