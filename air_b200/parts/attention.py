@@ -392,10 +392,11 @@ class Attention(TiledAttention, Mixer):
         bt = ctx.block_tables[pages.group]
         table = self.position.table()
         if self.eight and ctx.all_decode and H <= 16 * K:
-            # single next tokens: one launch, and the keys stream while the product ends
+            # single next tokens: one launch, and the keys stream while the product ends (those of another run's layer only behind it:
+            # that layer wrote its newest in this step)
             out = ops.empty((T, H, d), rt.dtype, x.device)
             ops.decode_attention8_fresh(qkv, self.bias, table, pages.kv, cache[1].scales, bt, ctx.token_seq, ctx.positions, out, H,
-                                        self.window, self.scale, write_kv=owns_cache, status=ctx.status, early=True)
+                                        self.window, self.scale, write_kv=owns_cache, status=ctx.status, early=owns_cache)
             return self._project(out.view(T, H * d), ctx)
         if self.eight:
             q = ops.empty((T, H, d), rt.dtype, x.device)

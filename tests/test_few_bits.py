@@ -99,3 +99,25 @@ def test_shapes_of_rows_in_four_bits():
 def test_what_a_report_says():
     r = LoadReport(in_four_bits={"a": 0.11, "b": 0.125})
     assert r.summary() == "2 matrices were rounded to microscaled 4-bit floating point, b the furthest: off by 12.5% of its root mean square"
+
+
+@pytest.mark.parametrize("owns", [True, False])
+def test_pages_of_another_run_are_read_behind_the_wait(owns, monkeypatch):
+    """A step of single tokens asks for old keys and values ahead of the q/k/v product's end only where none of them was written in
+    this step: not those of another run's layer."""
+    from air_b200.parts.attention import Attention
+    heads, kv_heads, d, T = 4, 2, 64, 3
+    part = object.__new__(Attention)
+    part.heads, part.kv_heads, part.head_dim, part.window, part.scale, part.bias, part.eight = heads, kv_heads, d, None, 0.125, None, True
+    part.rt = SimpleNamespace(dtype=torch.bfloat16, page_tokens=64, is_fp32=False)
+    part.position = SimpleNamespace(table=lambda: torch.zeros(8, d))
+    width = (heads + 2 * kv_heads) * d
+    product = lambda n: type("Product", (), {"small": lambda self, x: True, "partial": lambda self, x: torch.zeros(1, T, n),
+                                             "__call__": lambda self, x, dtype: torch.zeros(T, n, dtype=dtype)})()
+    part.qkv, part.q_only, part.o = product(width), product(heads * d), product(32)
+    seen = []
+    monkeypatch.setattr(ops, "empty", lambda shape, dtype, device: torch.empty(shape, dtype=dtype))
+    monkeypatch.setattr(ops, "decode_attention8_fresh", lambda *a, **kw: seen.append((kw["write_kv"], kw["early"])))
+    ctx = SimpleNamespace(all_decode=True, block_tables=[None], token_seq=None, positions=None, status=None)
+    part.forward(torch.zeros(T, 32), ctx, (SimpleNamespace(kv=None, group=0), SimpleNamespace(scales=None)), owns_cache=owns)
+    assert seen == [(owns, owns)]
