@@ -131,11 +131,12 @@ decode_attention_tma_kernel(const __grid_constant__ CUtensorMap map_cache, const
     // is done, see embedding_kernel) and keys and values of earlier steps; the token's own key and value never
     // come from the copy (they are patched into the tile from shared memory).  So the first tiles of old keys
     // are on their way while the product's last blocks still run.  Without fresh.qkv the token's key and value
-    // were written to the page by the predecessor itself, and everybody waits.
+    // were written to the page by the predecessor itself, and everybody waits; so they do where the pages are another run's
+    // (fresh.cache null), whose layer has written the token's key and value in this step.
     // alongside: see the head of this file; the first block alone waits, at its end, for all of the grid.
     // For the same reason everybody reads the token's place ahead of the wait then: two reads after one another that every
     // block's way to its first sums of the product would begin with.
-    if (!alongside && !fresh.qkv) pdl_wait();
+    if (!alongside && !fresh.cache) pdl_wait();
     const int t = blockIdx.z;
     const int slot = token_seq[t], pos = positions[t];
     const int lo = window > 0 ? max(0, pos - window + 1) : 0;

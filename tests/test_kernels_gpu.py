@@ -1262,3 +1262,29 @@ def test_products_of_few_rows_with_two_issuing_warps(K, T):
                 # (the slope of x / (1 + e^-x) is at most 1.1; the function and the scale themselves: 2^-19 of the result)
                 bound = 1.1 * dg * (u.abs() + du) + silu.abs() * du + (2.0 ** -8 + 2.0 ** -19) * (silu * u).abs() + 1e-30
                 assert ((out - silu * u).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("d,H,K,splits", [(128, 28, 4, None), (64, 4, 2, 1), (128, 8, 1, 3)])
+def test_fresh_decode_over_pages_that_the_launch_right_ahead_has_written(d, H, K, splits):
+    """Keys and values of another run (write_kv False): its layer's launches of this step are waited for."""
+    o, P, n = ops(), 64, 2000
+    g = torch.Generator().manual_seed(d + H)
+    pages = -(-n // P)
+    bt = torch.randperm(pages, generator=g).int().view(1, -1).cuda()
+    width = (H + 2 * K) * d
+    angle = torch.rand((n, d // 2), generator=g) * 6
+    table = torch.cat([angle.cos(), angle.sin()], 1).cuda()
+    every, zero = torch.arange(n, dtype=torch.int32).cuda(), torch.zeros(n, dtype=torch.int32).cuda()
+    last = every[-1:].contiguous()
+    q = torch.empty((n, H, d), dtype=torch.bfloat16, device="cuda")
+    cache = torch.zeros((pages, 2, K, P, d), dtype=torch.bfloat16, device="cuda")
+    rows = [torch.randn((n, width), generator=g).cuda() for _ in range(3)]
+    ones = [r[-1:].contiguous() for r in rows]
+    got, want = torch.empty((1, H, d), dtype=torch.bfloat16, device="cuda"), torch.empty((1, H, d), dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    for r, one in zip(rows, ones):
+        o.qkv_rope_store(r, None, table, every, zero, bt, q, cache, H, K, d)
+        o.decode_attention_fresh(one, None, table, cache, bt, zero[:1], last, got, H, None, d ** -0.5, write_kv=False, splits=splits)
+        torch.cuda.synchronize()
+        o.decode_attention_fresh(one, None, table, cache, bt, zero[:1], last, want, H, None, d ** -0.5, write_kv=False, splits=splits)
+        assert torch.equal(got, want)
