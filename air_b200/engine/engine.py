@@ -170,14 +170,17 @@ class Engine:
     @staticmethod
     def _pages_that_fit(model: Model, config: EngineConfig) -> int:
         """The pool's size from the memory that is left: free bytes (with the allocator's unused blocks given
-        back first) times memory_fraction, over what a page number costs in all runs; at most what
-        max_requests requests of the longest context could hold."""
+        back first) times memory_fraction, over what a page number costs in all runs, and besides in the one layer that takes
+        most for it while a step runs (CacheNeed.step_bytes); at most what max_requests requests of the longest context could hold."""
         torch.cuda.empty_cache()
         free, _ = torch.cuda.mem_get_info(model.rt.device)
         per_page = CacheManager.bytes_per_page(model.cache_needs(), config.page_tokens, model.rt.dtype)
         if per_page == 0:
             return 1
-        pages = int(free * config.memory_fraction) // per_page
+        paged = [need for needs in model.cache_needs() for need in needs if need.paged]
+        per_page += max(need.step_bytes(config.page_tokens, 0) for need in paged)
+        beside = max(need.step_bytes(0, config.max_requests) for need in paged)
+        pages = (int(free * config.memory_fraction) - beside) // per_page
         most = config.max_requests * -(-model.spec.max_positions // config.page_tokens)
         if pages < 1:
             raise RuntimeError(f"air_b200: {free >> 20} MiB of device memory are free after the weights, "

@@ -105,6 +105,11 @@ class CacheNeed:
             n *= s
         return n * torch.empty((), dtype=self.element_dtype(compute_dtype)).element_size()
 
+    def step_bytes(self, tokens: int, requests: int) -> int:
+        """Device bytes that a layer may take for a while, besides what is kept, in a step that sees `tokens` tokens of `requests`
+        requests."""
+        return 0
+
 
 @dataclass
 class PagedKVView:
@@ -159,6 +164,10 @@ class PagedKV8(CacheNeed):
 
     def element_dtype(self, compute_dtype):
         return torch.float8_e4m3fn
+
+    def step_bytes(self, tokens, requests):
+        # the bfloat16 copy of what portions see (ops.prefill_attention8), whole tiles of 64 tokens at either end of a request
+        return (tokens + 2 * 64 * requests) * 2 * self.kv_heads * self.head_dim * 2
 
     def view(self, tensor, group):
         return PagedKVView(tensor, group, self)

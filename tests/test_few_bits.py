@@ -121,3 +121,31 @@ def test_pages_of_another_run_are_read_behind_the_wait(owns, monkeypatch):
     ctx = SimpleNamespace(all_decode=True, block_tables=[None], token_seq=None, positions=None, status=None)
     part.forward(torch.zeros(T, 32), ctx, (SimpleNamespace(kv=None, group=0), SimpleNamespace(scales=None)), owns_cache=owns)
     assert seen == [(owns, owns)]
+
+
+@pytest.mark.parametrize("needs,copied", [([PagedKV8(4, 128)] * 2, 4 * 128), ([PagedKV8(2, 64, 100), PagedKV8(8, 128), PagedKV8(2, 64)], 8 * 128),
+                                          ([PagedKV(4, 128)] * 2, 0)])
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_the_pool_leaves_room_for_what_a_step_copies(needs, copied, page, monkeypatch):
+    """Every page seen by portions of one step, of as many requests as there may be, is copied to 16 bits, a layer at a time."""
+    free, requests = 40 << 30, 24
+    runs = [(n, n.scales) if isinstance(n, PagedKV8) else (n,) for n in needs]
+    model = SimpleNamespace(rt=SimpleNamespace(device=None, dtype=torch.bfloat16), cache_needs=lambda: runs,
+                            spec=SimpleNamespace(max_positions=1 << 30))
+    monkeypatch.setattr(torch.cuda, "empty_cache", lambda: None)
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device: (free, free))
+    pages = Engine._pages_that_fit(model, EngineConfig(page_tokens=page, max_requests=requests, max_tokens=None, memory_fraction=0.9))
+    kept = CacheManager.bytes_per_page(runs, page, torch.bfloat16)
+    # the worst case: requests of as many tokens as they hold, in tiles of 64, an unfinished one at either end
+    copy = lambda n: (n * page // 64 + 2 * requests) * 64 * 2 * copied * 2
+    assert pages * kept + copy(pages) <= 0.9 * free < (pages + 2) * kept + copy(pages + 2) + (1 << 20)
+
+
+def test_no_room_for_a_page(monkeypatch):
+    runs = [(PagedKV8(4, 128), PagedKV8(4, 128).scales)]
+    model = SimpleNamespace(rt=SimpleNamespace(device=None, dtype=torch.bfloat16), cache_needs=lambda: runs,
+                            spec=SimpleNamespace(max_positions=1024))
+    monkeypatch.setattr(torch.cuda, "empty_cache", lambda: None)
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device: (1 << 20, 1 << 30))
+    with pytest.raises(RuntimeError, match="a cache page takes"):
+        Engine._pages_that_fit(model, EngineConfig(max_requests=4, max_tokens=None))
