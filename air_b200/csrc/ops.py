@@ -2105,11 +2105,12 @@ def mxfp4_linear(x, w, w_scales, out, terms=1, splits=1, status=None, add=False,
                                                w.data_ptr(), w_scales.data_ptr(), out.data_ptr(), _DT[out.dtype], rows, n, k, terms,
                                                splits, *mode, 1 if w_ready else 0, _stream()), "mxfp4_linear")
         return out
-    memory = empty((_mxfp4_need(rows, n, k, terms, splits)[0],), torch.uint8, x.device)
+    need, joined = _mxfp4_need(rows, n, k, terms, splits)
+    memory = empty((need,), torch.uint8, x.device)
     global launches
     _check(_get("air_mxfp4_linear")(x.data_ptr(), _DT[x.dtype], memory.data_ptr(), w.data_ptr(), w_scales.data_ptr(), out.data_ptr(),
                                     _DT[out.dtype], rows, n, k, terms, splits, *mode, _stream()), "mxfp4_linear")
-    launches += 1
+    launches += 2 if splits == 1 and joined > 1 else 1      # (the rounding, and the sum of the parts)
     return out
 
 
@@ -2313,5 +2314,5 @@ def prefill_attention8(q, cache, scales, block_table, tiles, out, window, scale,
         0 if segments is None else segments.shape[0], _ptr(items) if n_items else None, n_items,
         int(slots) if segments is not None else 0, _ptr(part_o), _ptr(part_ml), out.data_ptr(), H, K, d, P, int(window or 0),
         float(scale), _ptr(status), _stream()), "prefill_attention8")
-    launches += 1
+    launches += 2 if n_items else 1      # (the copy, and the merge of the segments)
     return out

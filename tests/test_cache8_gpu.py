@@ -574,3 +574,16 @@ def test_a_tile_of_large_values_costs_the_others_no_bits(d, H, K, tile, splits, 
     largest = rows[1].abs().amax((1, 2)).repeat_interleave(H // K, 0)[None, :, None]
     tolerance = size * (2.0 ** -11 + 2.0 ** -16) + want.abs() * 2.0 ** -8 + largest * n * 2.0 ** -32
     assert ((out.cpu().double() - want).abs() <= tolerance * 1.01 + 1e-30).all()
+
+
+@pytest.mark.parametrize("count,before,kernels", [(40, 10, 2), (300, 5000, 3)])
+def test_launches_of_portions_are_counted(count, before, kernels):
+    d, P, H, K = 64, 64, 4, 2
+    pool = Pool([count + before], K, P, d, seed=50)
+    q = torch.zeros((count, H, d), dtype=torch.bfloat16, device="cuda")
+    plan = plan_portions([count], [before], pool.slots, H, None, "cuda")
+    assert (plan.items is not None and plan.items.shape[0] > 0) == (kernels == 3)
+    launched = ops.launches
+    ops.prefill_attention8(q, pool.cache, pool.scales, pool.table, plan.tiles, torch.empty_like(q), None, 0.1, segments=plan.segments,
+                           items=plan.items, slots=plan.slots)
+    assert ops.launches - launched == kernels
