@@ -114,13 +114,19 @@ def portion_tiles(n: int, pos0: int, slot: int, row0: int, window):
 
 def held_tiles(counts, lengths, slots, window):
     """int32 [pages, 4]: the 64-token tiles that portions of counts[i] tokens behind lengths[i] earlier ones of the requests in slots[i]
-    see, as ops.PortionTiles describes them."""
-    held = [np.zeros((0, 4), dtype=np.int32)]
+    see, as ops.PortionTiles describes them; of portions of one request, those of them all, each tile once (it has one place in
+    the copy, which the causal mask cuts for every row)."""
+    spans = {}
     for n, pos0, slot in zip(counts, lengths, slots):
-        lowest = max(0, pos0 - window + 1) if window else 0
-        tiles = np.arange(lowest // 64, (pos0 + n - 1) // 64 + 1, dtype=np.int32)
+        if n > 0:
+            lowest, end = max(0, pos0 - window + 1) if window else 0, pos0 + n
+            a, b = spans.get(slot, (lowest, end))
+            spans[slot] = (min(a, lowest), max(b, end))
+    held = [np.zeros((0, 4), dtype=np.int32)]
+    for slot, (lowest, end) in spans.items():
+        tiles = np.arange(lowest // 64, (end - 1) // 64 + 1, dtype=np.int32)
         rows = np.empty((tiles.shape[0], 4), dtype=np.int32)
-        rows[:, 0], rows[:, 1], rows[:, 2], rows[:, 3] = slot, tiles, lowest, pos0 + n
+        rows[:, 0], rows[:, 1], rows[:, 2], rows[:, 3] = slot, tiles, lowest, end
         held.append(rows)
     return np.concatenate(held)
 

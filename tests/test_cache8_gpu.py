@@ -587,3 +587,21 @@ def test_launches_of_portions_are_counted(count, before, kernels):
     ops.prefill_attention8(q, pool.cache, pool.scales, pool.table, plan.tiles, torch.empty_like(q), None, 0.1, segments=plan.segments,
                            items=plan.items, slots=plan.slots)
     assert ops.launches - launched == kernels
+
+
+@pytest.mark.parametrize("window", [None, 50])
+def test_several_portions_of_one_request(window):
+    d, P, H, K = 64, 32, 4, 2
+    counts, before, total = [64, 37, 1, 200], [10, 74, 111, 112], 312
+    pool = Pool([total, 90], K, P, d, seed=51)
+    poison(pool, pool.slots[0], total)
+    slots = [pool.slots[0]] * 4
+    q = (torch.randn((sum(counts) + 90, H, d), generator=pool.g) * 4).bfloat16()
+    out = torch.full(q.shape, math.nan, dtype=torch.bfloat16, device="cuda")
+    plan = plan_portions(counts + [90], before + [0], slots + [pool.slots[1]], H, window, "cuda")
+    ops.prefill_attention8(q.cuda(), pool.cache, pool.scales, pool.table, plan.tiles, out, window, d ** -0.5, segments=plan.segments,
+                           items=plan.items, slots=plan.slots)
+    for first, n, b, slot in ((0, 302, 10, pool.slots[0]), (302, 90, 0, pool.slots[1])):
+        want, size = attention64(q[first:first + n], torch.arange(b, b + n), pool.rows(slot, b + n), window, d ** -0.5)
+        tolerance = size * (2.0 ** -8 + 2 * 7.6e-5) + want.abs() * 2.0 ** -8          # (as for portions of several requests)
+        assert ((out[first:first + n].cpu().double() - want).abs() <= tolerance * 1.01 + 1e-30).all()

@@ -149,3 +149,9 @@ def test_no_room_for_a_page(monkeypatch):
     monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device: (1 << 20, 1 << 30))
     with pytest.raises(RuntimeError, match="a cache page takes"):
         Engine._pages_that_fit(model, EngineConfig(max_requests=4, max_tokens=None))
+
+
+def test_portions_of_one_request_share_its_tiles():
+    held = held_tiles([64, 37, 5, 0], [10, 74, 300, 7], [3, 3, 1, 2], 40).tolist()
+    assert held == [[3, 0, 0, 111], [3, 1, 0, 111], [1, 4, 261, 305]]
+    assert held_tiles([5, 64, 37], [300, 74, 10], [1, 3, 3], None).tolist() == [[1, t, 0, 305] for t in range(5)] + [[3, t, 0, 138] for t in range(3)]
