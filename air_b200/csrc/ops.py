@@ -2083,6 +2083,8 @@ def mxfp4_linear(x, w, w_scales, out, terms=1, splits=1, status=None, add=False,
         _req(x.ss, "x's sums of squares", (torch.float32,), (-(-k // PRENORM_CHUNK), rows))
         if rows > 64:
             raise KernelError("mxfp4_linear: rows of a norm short of their scale are taken up to 64")
+    if w.dim() not in (2, 3):
+        raise KernelError(f"mxfp4_linear: w has shape {tuple(w.shape)}")
     n = w.shape[-2]
     _req_mxfp4(w, w_scales, n, k, 1, "w")
     if splits > 1:
@@ -2129,6 +2131,11 @@ def _req_cache8(cache, scales, kv_heads=None):
         raise KernelError(f"pages of 8-bit numbers take multiples of {CACHE8_BLOCK} tokens, not {P}")
     _req(scales, "scales", (torch.float32,), (pages, 2, K, P // CACHE8_BLOCK))
     return K, P, d
+
+
+def _req_groups(heads, kv_heads):
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise KernelError(f"attention over pages of 8-bit numbers: {heads} query heads over {kv_heads}")
 
 
 def _req_batch(block_table, token_seq, positions, T):
@@ -2199,6 +2206,7 @@ def decode_attention8(q, cache, scales, block_table, token_seq, positions, out, 
     request, keys 0 .. position or the last `window` of them."""
     T, H, d = q.shape
     K, P, _ = _req_cache8(cache, scales)
+    _req_groups(H, K)
     _req(q, "q", (torch.bfloat16,), (T, H, cache.shape[4]))
     _req_batch(block_table, token_seq, positions, T)
     _req(out, "out", (torch.bfloat16,), (T, H, d))
@@ -2231,6 +2239,7 @@ def decode_attention8_fresh(qkv, bias, table, cache, scales, block_table, token_
     product that made qkv), and are read while that one ends."""
     K, P, d = _req_cache8(cache, scales)
     T, H = qkv.shape[-2], heads
+    _req_groups(H, K)
     width = (H + 2 * K) * d
     parts = 1 if qkv.dim() == 2 else qkv.shape[0]
     _req(qkv, "qkv", (torch.float32,), (T, width) if qkv.dim() == 2 else (parts, T, width))
@@ -2241,7 +2250,7 @@ def decode_attention8_fresh(qkv, bias, table, cache, scales, block_table, token_
     _req(out, "out", (torch.bfloat16,), (T, H, d))
     if not tile_pages(P):
         raise KernelError(f"decode_attention8_fresh: page size {P} is neither a divisor nor a multiple of 64")
-    if H % K or H // K > 16:
+    if H // K > 16:
         raise KernelError(f"decode_attention8_fresh: {H} heads over {K}: up to 16 to a key/value head are taken")
     least = 1
     if splits is None:
@@ -2279,6 +2288,7 @@ def prefill_attention8(q, cache, scales, block_table, tiles, out, window, scale,
     tiles, held = tiles
     T, H, d = q.shape
     K, P, _ = _req_cache8(cache, scales)
+    _req_groups(H, K)
     _req(q, "q", (torch.bfloat16,), (T, H, cache.shape[4]))
     _req(block_table, "block_table", _I32, (None, None))
     _req(tiles, "tiles", _I32, (None, 4))

@@ -605,3 +605,21 @@ def test_several_portions_of_one_request(window):
         want, size = attention64(q[first:first + n], torch.arange(b, b + n), pool.rows(slot, b + n), window, d ** -0.5)
         tolerance = size * (2.0 ** -8 + 2 * 7.6e-5) + want.abs() * 2.0 ** -8          # (as for portions of several requests)
         assert ((out[first:first + n].cpu().double() - want).abs() <= tolerance * 1.01 + 1e-30).all()
+
+
+@pytest.mark.parametrize("H,K", [(2, 4), (6, 4), (4, 0), (0, 4)])
+def test_heads_that_are_not_a_multiple_are_refused(H, K):
+    P, d = 64, 64
+    c = torch.zeros((3, 2, K, P, d), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    s = torch.ones((3, 2, K, P // 16), device="cuda")
+    bt = torch.zeros((1, 2), dtype=torch.int32, device="cuda")
+    q = torch.zeros((1, H, d), dtype=torch.bfloat16, device="cuda")
+    pos, seq = batch([1], [5], [0])
+    plan = plan_portions([1], [5], [0], max(H, 1), None, "cuda")
+    for call in (lambda: ops.decode_attention8(q, c, s, bt, seq, pos, torch.empty_like(q), None, 1.0),
+                 lambda: ops.decode_attention8(q, c, s, bt, seq, pos, torch.empty_like(q), None, 1.0, splits=2),
+                 lambda: ops.prefill_attention8(q, c, s, bt, plan.tiles, torch.empty_like(q), None, 1.0),
+                 lambda: ops.decode_attention8_fresh(torch.zeros((1, (H + 2 * K) * d), device="cuda"), None, rotation(8, d).cuda(), c, s, bt, seq, pos,
+                                                     torch.empty_like(q), H, None, 1.0)):
+        with pytest.raises(ops.KernelError):
+            call()
