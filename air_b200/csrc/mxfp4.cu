@@ -315,7 +315,7 @@ mxfp4_add_prenorm_kernel(float* __restrict__ h, const TD* __restrict__ delta, in
 template <typename T>
 __global__ void __launch_bounds__(MXQ_THREADS)
 mxfp4_values_kernel(const uint32_t* __restrict__ packed, const uint8_t* __restrict__ scales, T* __restrict__ out, int rows, int k) {
-    pdl_enter();
+    pdl_enter(TR_MXFP4_VALUES);
     const uint32_t line = blockIdx.x, col = (blockIdx.y * blockDim.x + threadIdx.x) * 16, row = line % rows, t = line / rows, j = col / 32;
     if (col >= k) return;
     const size_t row_tiles = (rows + 127) / 128, k_tiles = 2 * ((k + 255) / 256);
@@ -702,7 +702,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_consta
 template <typename TO>
 __global__ void __launch_bounds__(256)
 mxfp4_join_kernel(const float* __restrict__ parts, TO* __restrict__ out, size_t n, int n_parts, int mode, float alpha, float limit, float shift) {
-    pdl_enter();
+    pdl_enter(TR_MXFP4_JOIN);
     const size_t at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 2;
     if (at >= n) return;
     const bool both = at + 1 < n;

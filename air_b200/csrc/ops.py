@@ -188,13 +188,15 @@ TRACE_NAMES = {1: "embedding", 2: "add_rmsnorm", 3: "qkv_rope_store", 4: "silu_m
                12: "gemm_tc", 13: "sample", 14: "short_conv", 15: "linear_scan", 16: "gated_rmsnorm",
                17: "qkv_prepare", 18: "glu", 19: "scaled_norm", 20: "post_norm", 21: "qk_normed_prepare",
                22: "latent_prepare", 23: "moe_route", 24: "moe_sort", 25: "grouped_gemm", 26: "gather_keys", 27: "masked_softmax", 28: "grouped_attention", 29: "polynorm", 30: "stream_add", 31: "head_gate",
-               32: "normed_add_norm", 33: "relu2", 34: "stream_norm", 35: "residual_conv", 36: "mlstm", 37: "turn_heads"}
+               32: "normed_add_norm", 33: "relu2", 34: "stream_norm", 35: "residual_conv", 36: "mlstm", 37: "turn_heads",
+               38: "mxfp4_values", 39: "mxfp4_join"}
 
 
 def set_trace(buffer: Optional[torch.Tensor]) -> None:
     """buffer: int64 CUDA tensor of 1 + 2 * 16384 elements (zeroed), or None to stop tracing.  While set,
     block 0 of every kernel appends (kernel id, GPU nanosecond timer) after its wait on its predecessor;
-    element 0 counts the entries.  Differences of consecutive times are the kernels' spans in a graph."""
+    element 0 counts the entries.  Differences of consecutive times are the kernels' spans in a graph.  (The rounding to 4 bits and
+    the products in 4 bits make no entry: it cost them 0.1 us each.)"""
     lib = build.library()
     ptr = None if buffer is None else buffer.data_ptr()
     for src in build.sources():
