@@ -158,9 +158,9 @@ struct Fresh8 {
 };
 
 // GROUPS: of eight heads that a block takes, 1 or 2.  FEW: the grid is no larger than two blocks an SM, which then have six stages each
-// and registers for as many; of a larger one four share an SM, with three.  us with six stages and with three: one of 512 7.4 / 8.1, of
-// 2,048 8.3 / 9.9; 16 of 512 9.8 / 11.9, of 2,048 14.8 / 16.0; 64 of 100 to 8,192 73 / 63, 256 of 200 30 / 22 (from there on it is
-// the number of warps that counts: 393 instructions for a warp's 16 keys, most of them behind one another).
+// and registers for as many; of a larger one four share an SM, with three.  us with six stages and with three: one of 512 7.4 / 7.8, of
+// 2,048 8.4 / 9.5; 16 of 512 9.2 / 11.3, of 2,048 13.9 / 19.0; 64 of 100 to 8,192 75 / 64, 256 of 200 28 / 20 (from there on it is
+// the number of warps that counts: some 350 instructions for a warp's 16 keys, most of them behind one another).
 template <int D, int GROUPS, bool FRESH, bool FEW>
 __global__ void __launch_bounds__(D8_THREADS, GROUPS == 1 && !FEW ? 4 : 2)
 decode_attention8_kernel(const __grid_constant__ CUtensorMap map_cache, const Fresh8 fresh, const float* __restrict__ scales, const __nv_bfloat16* __restrict__ q,

@@ -21,8 +21,9 @@ namespace air {
 // that lets it become resident while its predecessor in the stream is still running, and every
 // kernel begins with pdl_enter(): it first tells the scheduler that its own successor may be
 // launched, then waits until its predecessor has completed and its writes are visible.  Whatever
-// a kernel does before pdl_enter() (setting up barriers, fetching weights, which no kernel
-// writes) overlaps the predecessor's tail.  Without the attribute both instructions do nothing.
+// a kernel does before pdl_enter() (setting up barriers, fetching weights, which no kernel of a
+// step writes; those that a caller may have rounded right ahead are waited for, mxfp4.cu)
+// overlaps the predecessor's tail.  Without the attribute both instructions do nothing.
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Optional timeline: when a trace buffer is set (air_set_trace), block 0 of every kernel appends

@@ -417,7 +417,7 @@ AIR_API int air_gemm_f32(const float* A, const float* W, const float* bias, floa
     }
     // From 64 steps of k on, a cluster with a block for every range: tiles of 64 x 64 wherever they share out as evenly over the
     // SMs as tiles of 32 x 64 do, whose outputs cost an eighth more to feed.  (32 rows by 16,384 x 2,048: 72 us against 117; 300 by
-    // 3,072 x 2,048: 119 against 111.  Tiles of 128 columns or rows were within 3 % of 64 x 64 at 512 and 2,048 rows and slower
+    // one of as many numbers a row that does not share out so: 119 against 111.  Tiles of 128 columns or rows were within 3 % of 64 x 64 at 512 and 2,048 rows and slower
     // below.)
     if (K >= 1024) {
         if (fullest(M, N, 32, 64, PARTS) * 1.125 < fullest(M, N, 64, 64, PARTS))

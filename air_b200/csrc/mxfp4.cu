@@ -1024,7 +1024,11 @@ static int launch_mxfp4_pair(const MxCall& c) {
 // Measured, us, tiles of 128 and of 256 tokens: 2,048 x 37,888 x 3,584 125 / 104, two terms 179 / 173, three 252 / 256; 2,048 x 5,120 x
 // 13,824 80 / 73, 120 / 134, 177 / 198.  One part and several: 128 x 640 x 2,048 6.6 / 7.0 (8), 128 x 4,608 x 3,584 8.0 / 9.5 (4), 256 x
 // 5,120 x 13,824 18.6 / 20.4 (3), 129 of them 18.5 / 17.4; 301 x 3,584 x 18,944 in two terms 34.5 / 32.6 (3), 128 x 3,584 x 18,944 in one
-// 14.9 with five.
+// 14.9 with five.  Few rows in two terms, their rounding included, with 1, 2, 4, 5, 7 and 8 parts (- where one would have no step), what is taken
+// in brackets: 1 x 4,608 x 3,584 8.0, 7.1, [6.5], 7.0, 6.7, -; 8 of them 8.2, 7.5, [6.7], 7.2, 6.8, -; 64 [9.2], 9.1, 8.4, 9.6, 9.0, -; 1 x 3,584 x
+// 3,584 8.1, 7.3, 6.4, [6.4], 6.8, -; 1 x 640 x 2,048 [6.2], 6.2, 5.7, -, -, 5.2; 64 of them [6.9], 6.9, 6.5, -, -, 6.2; 1 x 3,584 x 18,944 26.4, 16.6,
+// 11.2, [10.2], 12.3, 11.7; 64 of them 30.9, 20.5, 15.2, [13.8], 18.0, 17.6; 1 x 512 x 8,192 13.5, 9.6, 7.6, 7.3, 6.6, 6.5, [6.4 (16)]: within a fifth of
+// the best of them.
 struct MxPlan {
     int tn, pair, parts;
 };

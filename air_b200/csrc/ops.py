@@ -1713,7 +1713,7 @@ def asked_ahead(tensors):
     together.  Nothing where these do not hold the first one: the product right behind gains little from part of its matrix, and
     the one after it, which gains most, would get nothing.  Measured, a decoder layer in a chain of layers, us without and with 24 MB
     asked for, 1 or 2 requests of 40 to 100 tokens / 4 of 300: width 2,048 (8 MB of output matrix) 41.9 / 43.4 -> 40.3 / 41.8, 1,536
-    39.0 / 42.2 -> 38.8 / 41.4, 2,560 51.9 / 52.9 -> 51.9 / 53.0, 3,072 (19 MB) 52.5 / 54.6 -> 52.6 / 54.4; 3,584 (26 MB) 89.1 / 90.3 -> 89.6 /
+    39.0 / 42.2 -> 38.8 / 41.4, 2,560 51.9 / 52.9 -> 51.9 / 53.0; 3,584 (26 MB) 89.1 / 90.3 -> 89.6 /
     91.1 and 8 of 60 90.4 -> 91.3, 4,096 (34 MB) 85.7 / 87.5 -> 86.1 / 87.3, 5,120 102.0 / 104.0 -> 102.2 / 103.5; from 32 requests on the same either way."""
     tensors, left, asked = tensors[:2], AHEAD_BYTES, []
     if tensors and tensors[0].numel() * tensors[0].element_size() > left:
@@ -2191,10 +2191,10 @@ def cache8_rows(cache, scales, block_table, slots, lengths, out):
 def decode_splits8(tokens: int, heads: int, kv_heads: int):
     """(splits, 64-key tiles that one takes at least) for decode_attention8: for few requests as many blocks as stand on the SMs at once,
     two each (attention_decode8.cu), for more some 1,024 of eight tiles at least: unlike lengths want many splits, equal ones few.
-    Measured, us, with (2, 8), (4, 8), (8, 8): 64 requests of 100 to 8,192 tokens in any order, 28 heads over 4: 77, 72, 71; 60 of 100 and
-    four of 8,192: 61, 39, 33; 64 of 8,192: 91, 96, 100; 64 of 2,048: 32, 35, 42; 64 of 512: 19, 19, 20.  32 of 2,048 with 2 splits (on two
-    blocks an SM) and with 4 20.8 and 21.1, of 100 to 8,192 45 and 39.  16 of 2,048 with 2, 4 and 8: 19.8, 14.8, 19.5; one of 2,048 with
-    4 and 32: 10.8, 8.3."""
+    Measured, us, with (2, 8), (4, 8), (8, 8): 64 requests of 100 to 8,192 tokens in any order, 28 heads over 4: 80, 70, 65; 60 of 100 and
+    four of 8,192: 56, 46, 33; 64 of 8,192: 94, 99, 102; 64 of 2,048: 33, 37, 43; 64 of 512: 19, 19, 20.  32 of 2,048 with 2 splits (on two
+    blocks an SM) and with 4 20.2 and 20.1, of 100 to 8,192 52 and 43.  16 of 2,048 with 2, 4 and 8: 19.2, 14.0, 14.8; one of 2,048 with
+    4 and 32: 11.0, 8.4."""
     blocks = tokens * kv_heads * -(-(heads // kv_heads) // (8 if heads // kv_heads <= 8 else 16))
     if blocks > 128:
         return max(1, min(32, round(1024 / blocks))), 8
@@ -2238,7 +2238,8 @@ def decode_attention8_fresh(qkv, bias, table, cache, scales, block_table, token_
     """qkv_rope_store8 followed by decode_attention8 in one launch, for one token per request and up to 16 query heads to a key/value
     head: qkv float32 [T, (H + 2K) d] or [parts, T, (H + 2K) d], bias float32 or None, table float32 [positions, d]; the pages end up as
     qkv_rope_store8 leaves them.  early: pages, scales, tables and positions were written before the launch right ahead started (the
-    product that made qkv), and are read while that one ends."""
+    product that made qkv), and are read while that one ends; so it is where a step writes to these pages by this call alone, and not with
+    write_kv False, where another layer of the step has written them."""
     K, P, d = _req_cache8(cache, scales)
     T, H = qkv.shape[-2], heads
     _req_groups(H, K)
